@@ -24,8 +24,10 @@
 // power of two into f16's range.  The value scale joins the exponent: with s the score in the exp2
 // domain and e the exponent of V's scale,
 //   P = 2^(s + e - m),   O = sum P v8,   l = sum P 2^-e,   m = running max of s + e,   out = O / l,
-// which is softmax(s) V for any m, and P <= 1 whatever the scales, so f16 holds it (2^-12 relative; a
-// weight below 2^-14 of the largest is held to 2^-25 of it).  S, m, l and O are fp32.
+// which is softmax(s) V for any m, so parts with other references (a prefix's, whose m is max s) join by
+// the same formula.  With m the maximum of the pages' own s + e, P <= 1 reaches 1 whatever the scales, so
+// f16 holds it: 2^-12 relative, and P v8 below 2^-14 of the largest to 2^-25 of it.  S, m, l and O are fp32
+// (a token counts as nothing where its s + e is 126 below the largest).
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp16.h>
@@ -481,34 +483,6 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 ? 3 : 2)
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(unit_empty);
-    // The prefix's parts, where there are any, are where the warps' sums begin (every fourth part each).
-    if (x.done > 0 && p == 0) {
-      const int parts = prefix_parts(args, x.done);
-      for (int i = warp; i < parts; i += kWarps)
-#pragma unroll
-        for (int u = 0; u < kTiles; ++u)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int r = 8 * u + 2 * t + j;
-            if (r >= rows) continue;
-            const long long part =
-                i * args.part_rows + ((long long)(v / args.tiles) * args.Hkv + h) * args.G + r;
-            const float2 ml = *reinterpret_cast<const float2*>(args.part_ml + part * 2);
-            float2 po[8];
-#pragma unroll
-            for (int c = 0; c < 8; ++c)
-              po[c] = *reinterpret_cast<const float2*>(args.part_o + part * kKvDim + 16 * c + 2 * g);
-            const float M = fmaxf(m_r[u][j], ml.x);
-            const float fo = part_factor(m_r[u][j], M), fp = part_factor(ml.x, M);
-            m_r[u][j] = M;
-            l_r[u][j] = fmaf(g == 0 ? ml.y : 0.f, fp, l_r[u][j] * fo);   // a row's lanes are summed at the end
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              o[u][c][j] = fmaf(po[c].x, fp * 0x1p60f, o[u][c][j] * fo);
-              o[u][c][2 + j] = fmaf(po[c].y, fp * 0x1p60f, o[u][c][2 + j] * fo);
-            }
-          }
-    }
     const int all_see = min(len, x.pos0 + 1);          // every row sees the keys below
     const int half = (warp & 1) * 32;
 
@@ -651,6 +625,35 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 ? 3 : 2)
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[s]);
+    }
+    // The prefix's parts, where there are any (every fourth part each).  Only now: their m is a maximum
+    // of s, without V's exponents, and would put a page's P out of f16's range where those are small.
+    if (x.done > 0 && p == 0) {
+      const int parts = prefix_parts(args, x.done);
+      for (int i = warp; i < parts; i += kWarps)
+#pragma unroll
+        for (int u = 0; u < kTiles; ++u)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int r = 8 * u + 2 * t + j;
+            if (r >= rows) continue;
+            const long long part =
+                i * args.part_rows + ((long long)(v / args.tiles) * args.Hkv + h) * args.G + r;
+            const float2 ml = *reinterpret_cast<const float2*>(args.part_ml + part * 2);
+            float2 po[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              po[c] = *reinterpret_cast<const float2*>(args.part_o + part * kKvDim + 16 * c + 2 * g);
+            const float M = fmaxf(m_r[u][j], ml.x);
+            const float fo = part_factor(m_r[u][j], M), fp = part_factor(ml.x, M);
+            m_r[u][j] = M;
+            l_r[u][j] = fmaf(g == 0 ? ml.y : 0.f, fp, l_r[u][j] * fo);   // a row's lanes are summed at the end
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              o[u][c][j] = fmaf(po[c].x, fp * 0x1p60f, o[u][c][j] * fo);
+              o[u][c][2 + j] = fmaf(po[c].y, fp * 0x1p60f, o[u][c][2 + j] * fo);
+            }
+          }
     }
 #pragma unroll
     for (int u = 0; u < kTiles; ++u)
