@@ -55,15 +55,19 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[16], int at) {
 
 // (a b - c d) (r_hi + r_lo) rounded to odd: the last bit is set where anything is left over, so that
 // rounding it once more, to e4m3, gives what rounding the exact value would (a rounding to nearest
-// first could end on a tie that the exact value is not on).
+// first could end on a tie that the exact value is not on).  Where the products nearly cancel, or with
+// the factor's second half, the remainders come to several units of the product y: they are added to
+// it, exactly, before the last bit is looked at.  (Dekker's sum: exact unless `more` is the larger of the
+// two, for which s has to be below 2^-22 of its products; such a value of a rotated pair is code 0.)
 __device__ __forceinline__ float rotate_sticky(float a, float b, float c, float d, float r_hi, float r_lo) {
   // (Intrinsics: a product contracted into the next sum would not be the one whose error is taken.)
   const float p = __fmul_rn(a, b), q = __fmul_rn(c, d);
   const float s = __fsub_rn(p, q), t = __fsub_rn(s, p);
   const float rest = __fadd_rn(__fsub_rn(__fsub_rn(p, __fsub_rn(s, t)), __fadd_rn(q, t)),
                                __fsub_rn(fmaf(a, b, -p), fmaf(c, d, -q)));
-  const float y = __fmul_rn(s, r_hi);
-  const float left = fmaf(s, r_hi, -y) + fmaf(s, r_lo, rest * r_hi);
+  const float y0 = __fmul_rn(s, r_hi);
+  const float more = fmaf(s, r_hi, -y0) + fmaf(s, r_lo, rest * r_hi);
+  const float y = __fadd_rn(y0, more), left = __fsub_rn(more, __fsub_rn(y, y0));
   const uint32_t bits = __float_as_uint(y);
   // (No remainder of infinities and NaN: both comparisons are false.)
   if ((bits & 1u) == 0 && y != 0.f && (left > 0.f || left < 0.f))
