@@ -82,6 +82,7 @@ struct Args {
   const int* seq_lens;     // context length incl. the queries
   const int* cu_q;         // [B + 1] query offsets, or null: one query per sequence
   int num_q;               // rows of q
+  int max_q;               // queries of a sequence at most (with cu_q)
   const uint8_t* scales;
   int G, Hkv;
   int num_pages, max_pages;   // of the cache; columns of the block table
@@ -126,7 +127,8 @@ __device__ __forceinline__ Tile tile_of(const Args& a, int v) {   // v = sequenc
   x.len = min(a.seq_lens[b], a.max_pages * kKvPage);
   const int q_begin = a.cu_q != nullptr ? a.cu_q[b] : b;
   int q_len = a.cu_q != nullptr ? a.cu_q[b + 1] - q_begin : 1;
-  if (q_begin < 0 || q_len < 0 || q_len > a.num_q - q_begin) {   // offsets outside q: no queries
+  // Offsets outside q, or more queries than the launch has tiles for: no queries.
+  if (q_begin < 0 || q_len < 0 || q_len > a.num_q - q_begin || q_len > a.max_q) {
     raise_status(a.status, kStatusBadArgument);
     q_len = 0;
   }
@@ -915,6 +917,7 @@ void attn_fp8(const char* what, const at::Tensor& q, const at::Tensor& k_cache, 
   a.seq_lens = seq_lens.data_ptr<int>();
   a.cu_q = cu_q;
   a.num_q = static_cast<int>(q.size(0));
+  a.max_q = static_cast<int>(max_q_len);
   a.prefix_len = prefix_len;
   a.part_o = part_o;
   a.part_ml = part_ml;
@@ -925,9 +928,11 @@ void attn_fp8(const char* what, const at::Tensor& q, const at::Tensor& k_cache, 
   a.G = static_cast<int>(q.size(1)) / a.Hkv;
   a.num_pages = static_cast<int>(k_cache.size(0));
   a.max_pages = static_cast<int>(block_table.size(1));
-  const bool narrow = a.G * max_q_len <= 8;   // one group of eight rows holds a sequence's
+  // (At least a tile, which looks at the offsets, if there are to be no queries.)
+  const int64_t queries = std::max<int64_t>(1, max_q_len);
+  const bool narrow = a.G * queries <= 8;   // one group of eight rows holds a sequence's
   a.tokens_per_tile = (narrow ? 8 : kMaxRows) / a.G;
-  const int64_t tiles = (max_q_len + a.tokens_per_tile - 1) / a.tokens_per_tile;
+  const int64_t tiles = (queries + a.tokens_per_tile - 1) / a.tokens_per_tile;
   TORCH_CHECK(B * tiles * a.Hkv < (1LL << 31), what, ": too many query tiles");
   a.tiles = static_cast<int>(tiles);
   a.units = static_cast<int>(B * tiles * a.Hkv);

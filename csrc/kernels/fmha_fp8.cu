@@ -110,6 +110,7 @@ struct Args {
   const int* cu_q;         // [B + 1]; null: one sequence of num_q queries that all see the prefix
   const int* prefix_len;   // [1] tokens, with cu_q null: its whole pages are the keys
   int num_q;               // rows of q
+  int max_q;               // queries of a sequence at most (with cu_q)
   int G, Hkv, Hq;
   int num_pages, max_pages;   // of the cache; columns of the block table
   int tokens_per_tile;     // 128 / G
@@ -232,8 +233,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();  // q, the cache and the lengths come from earlier kernels
   const int q_begin = kPrefill ? args.cu_q[b] : 0;
   const int asked = kPrefill ? args.cu_q[b + 1] - q_begin : args.num_q;
-  const bool inside = q_begin >= 0 && asked >= 0 && asked <= args.num_q - q_begin;
-  const int q_len = inside ? asked : 0;   // offsets outside q: no queries (and the status, below)
+  const bool inside = q_begin >= 0 && asked >= 0 && asked <= args.num_q - q_begin && asked <= args.max_q;
+  const int q_len = inside ? asked : 0;   // offsets outside q, or too many: no queries (and the status, below)
   // The row of the block table, and the tokens that count.
   int table_row = b, kv_len = 0;
   if constexpr (kPrefill) {
@@ -698,6 +699,7 @@ void launch(const char* what, const at::Tensor& q, const at::Tensor& k_cache, co
   a.Hq = static_cast<int>(q.size(1));
   a.G = a.Hq / a.Hkv;
   a.num_q = static_cast<int>(q.size(0));
+  a.max_q = static_cast<int>(max_q);
   a.num_pages = static_cast<int>(k_cache.size(0));
   a.max_pages = static_cast<int>(block_table.size(1));
   a.tokens_per_tile = kBM / a.G;
@@ -760,7 +762,8 @@ at::Tensor paged_prefill_fp8(const at::Tensor& q, const at::Tensor& k_cache, con
   TORCH_CHECK(cu_q.device() == q.device() && cu_q.scalar_type() == at::kInt && cu_q.is_contiguous() &&
                   cu_q.numel() == B + 1,
               what, ": cu_q must be contiguous int32 [B + 1] beside q");
-  if (B == 0 || q.size(0) == 0 || max_q_len <= 0) return out;
+  TORCH_CHECK(max_q_len >= 0 && max_q_len < (1LL << 31), what, ": max_q_len must not be negative");
+  if (B == 0 || q.size(0) == 0) return out;
   c10::cuda::CUDAGuard guard(q.device());
   // Runs of up to kShortRows rows of a KV head go through the decode kernel.
   if (max_q_len * G <= kShortRows) {

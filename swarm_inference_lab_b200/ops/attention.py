@@ -90,7 +90,8 @@ def paged_prefill_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     """:func:`paged_prefill` over an e4m3 cache: causal, packed q [T, Hq, 128] with int32 offsets
     ``cu_q`` [B+1]; the queries of a sequence are the last tokens of its context, ``max_q_len`` at
     most.  Rows of ``out`` behind the last sequence are left as they were; a query that sees no
-    key gets zeros; offsets outside ``q`` raise the device status."""
+    key gets zeros.  Offsets outside ``q``, or of more than ``max_q_len`` queries, raise the device
+    status, and the sequence's rows are left as they were."""
     return ext().paged_prefill_fp8(q, k_cache, v_cache, kv_scales, block_table, seq_lens, cu_q,
                                    max_q_len, out, SCALE_128 if scale is None else scale,
                                    get_workspace(q.device).status)
