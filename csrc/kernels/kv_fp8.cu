@@ -135,13 +135,12 @@ __global__ void __launch_bounds__(kThreads, 4) rope_kv_write_fp8_kernel(const Wr
       raw[i][0] = *reinterpret_cast<const uint4*>(row + i * kKvDim);
       raw[i][1] = *reinterpret_cast<const uint4*>(row + i * kKvDim + 64);
     }
-  const bool pos_ok = static_cast<unsigned>(pos) < static_cast<unsigned>(a.max_pos);
-  const bool slot_ok = slot < a.num_slots;
-  if (!(pos_ok && slot_ok)) {
+  // A token with a position or a slot outside is not written at all.
+  if (static_cast<unsigned>(pos) >= static_cast<unsigned>(a.max_pos) || slot >= a.num_slots) {
     if (lane == 0) raise_status(a.status, kStatusBadArgument);
-    if (!pos_ok) return;
+    return;
   }
-  const bool store = slot_ok && slot >= 0;
+  const bool store = slot >= 0;
   float c[8], s[8];
   if (h0 < a.Hq + a.Hkv) {
     const float* cs = a.cos_sin + (long long)pos * kKvDim + 8 * lane;
