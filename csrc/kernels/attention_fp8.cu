@@ -698,6 +698,7 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 ? 3 : 2)
     if (warp >= 2) put(warp - 2);
     const bool clean = consumers_agree(alive);
     if (warp < 2) take(warp);
+    __syncwarp();   // every lane of warp 1 has read slot 1
     if (warp == 1) put(1);
     named_bar_sync(1, kWarps * 32);
     if (warp == 0) {
