@@ -170,7 +170,8 @@ class LLMEngine:
         shares = 0 < n < len(prompt) and list(prompt[:n]) == self._prefix
         self.scheduler.admit(SeqRequest(rid, list(prompt), params.max_new_tokens,
                                         time.monotonic_ns(), stop_token_ids=params.stop_token_ids,
-                                        sampling=sampling, prompt_consumed=n if shares else 0))
+                                        sampling=sampling, prompt_consumed=n if shares else 0,
+                                        shared_tokens=n if shares else 0))
         if shares:
             self.kv.fork_prefix(_PREFIX, rid, n)
             self._sharing.add(rid)

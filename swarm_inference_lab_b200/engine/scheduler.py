@@ -46,6 +46,7 @@ class SeqRequest:
     first_token_ns: int = 0
     finish_ns: int = 0
     sampling: object | None = None   # SamplingParams of a non-greedy request (None: greedy)
+    shared_tokens: int = 0           # prompt tokens in whole pages that are there already (a shared prefix)
 
     @property
     def prefill_complete(self) -> bool:
@@ -111,6 +112,8 @@ class ContinuousScheduler:
             raise ValueError(f"duplicate request {req.request_id!r}")
         if len(req.prompt) == 0 or req.max_new_tokens <= 0:
             raise ValueError("prompt and max_new_tokens must be positive")
+        if not 0 <= req.shared_tokens <= len(req.prompt) or req.shared_tokens % self.page:
+            raise ValueError("shared_tokens must be whole pages of the prompt")
         if self._reserve_tokens(req) > self.kv_capacity:
             raise ValueError(f"request needs {self._reserve_tokens(req)} KV tokens, capacity "
                              f"{self.kv_capacity}")
@@ -118,7 +121,7 @@ class ContinuousScheduler:
         self.waiting.append(req)
 
     def _reserve_tokens(self, req: SeqRequest) -> int:
-        total = len(req.prompt) + req.max_new_tokens
+        total = len(req.prompt) + req.max_new_tokens - req.shared_tokens
         return ((total + self.page - 1) // self.page) * self.page
 
     @property

@@ -183,3 +183,23 @@ def test_cli_refuses_other_cache_types():
     from swarm_inference_lab_b200.cli import app
     r = CliRunner().invoke(app, ["run", "tiny-llama-gpu", "--kv-dtype", "int8"])
     assert r.exit_code != 0 and "kv-dtype" in r.output + str(r.exception)
+
+
+def test_a_request_on_a_shared_prefix_is_charged_its_own_pages():
+    """2560 shared tokens of 4096 and 1536 of room: requests of 2560 + 10 tokens need one page each."""
+    from swarm_inference_lab_b200.engine.scheduler import ContinuousScheduler, SeqRequest
+    sch = ContinuousScheduler(max_batch=64, prefill_token_budget=8192, kv_capacity_tokens=4096 - 2560)
+    for i in range(30):
+        sch.admit(SeqRequest(f"r{i}", list(range(2570)), 5, i, prompt_consumed=2560, shared_tokens=2560))
+    it = sch.next_iteration()
+    assert [n for _, n in it.prefill] == [10] * 24 and len(sch.waiting) == 6       # 24 pages are free
+    assert sch.reserved_tokens == 24 * 64
+    for rid, n in it.prefill:
+        sch.mark_prefill(rid, n, 1)
+    assert sch.reserved_tokens == 24 * 64                                          # not less as the prompt is taken in
+    with pytest.raises(ValueError, match="KV tokens"):
+        sch.admit(SeqRequest("own", list(range(2570)), 5, 99))
+    with pytest.raises(ValueError, match="shared"):
+        sch.admit(SeqRequest("odd", list(range(200)), 5, 99, shared_tokens=100))
+    with pytest.raises(ValueError, match="shared"):
+        sch.admit(SeqRequest("all", list(range(128)), 5, 99, shared_tokens=192))

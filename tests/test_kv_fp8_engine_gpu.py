@@ -186,3 +186,36 @@ def test_rows_of_a_sequence():
         # the bf16 rows are rounded themselves
         amax = b.abs().amax(-1, keepdim=True)
         assert ((a - b).abs() <= 2.0 ** -4 * b.abs() + 2.0 ** -10 * 2 * amax / 448 + 2.0 ** -8 * amax).all()
+
+
+def _tiny(moe=False, **kw):
+    from swarm_inference_lab_b200.engine.engine import LLMEngine
+    from swarm_inference_lab_b200.models.config import TINY_LLAMA_GPU, ModelConfig
+    from swarm_inference_lab_b200.models.dense import DenseWeights, TPInfo
+    from swarm_inference_lab_b200.models.moe import MoEWeights
+    cfg, weights = TINY_LLAMA_GPU, DenseWeights
+    if moe:
+        cfg, weights = ModelConfig(name="tiny-moe", family="qwen3_moe", vocab_size=2048, hidden_size=512, num_layers=2,
+                                   num_heads=4, num_kv_heads=2, head_dim=128, intermediate_size=1024, qk_norm=True,
+                                   num_experts=8, num_experts_per_tok=2, moe_intermediate_size=256,
+                                   rms_norm_eps=1e-6), MoEWeights
+    return LLMEngine(cfg, device="cuda", weights=weights.random(cfg, TPInfo(), "cuda", seed=3, std=0.06), **kw)
+
+
+def test_a_prefix_over_half_the_cache_serves_requests_together():
+    """The prefix's pages are there once: a request on them needs its own pages only."""
+    from swarm_inference_lab_b200.engine.engine import SamplingParams
+    eng = _tiny(max_batch=8, max_seq_len=3000, kv_pages=64, kv_dtype="fp8")
+    prefix = _prompts([40 * PAGE])[0]
+    assert eng.set_shared_prefix(prefix) == 40 * PAGE
+    prompts = [prefix + t for t in _prompts([10, 60, 1, 100, 5, 6, 7, 8])]
+    for p in prompts:
+        eng.add_request(p, SamplingParams(max_new_tokens=5))
+    assert len(eng.step()) == 8                                # all of them are admitted at once
+    assert eng.kv.alloc.free == 24 - 10                        # (two need two pages)
+    with pytest.raises(ValueError, match="KV tokens"):         # one that does not share has 24 pages
+        eng.add_request(_prompts([24 * PAGE])[0], SamplingParams(max_new_tokens=1))
+    while eng.scheduler.has_work():
+        eng.step()
+    _check_status()
+    assert eng.kv.alloc.free == 24
