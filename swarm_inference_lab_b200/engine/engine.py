@@ -128,26 +128,36 @@ class LLMEngine:
         """Prefill the whole pages (64 tokens) of ``tokens`` once and let every later request whose
         prompt begins with them, and goes on, start on those pages.  A decode batch of such requests
         attends to the prefix once for all (e4m3 cache).  Returns how many tokens are shared;
-        ``[]`` gives the pages back.  Only while no request is queued or running."""
+        ``[]`` gives the pages back, and so does a call whose prefill fails.  Only while no request is
+        queued or running."""
         if self.scheduler.has_work():
             raise ValueError("set the shared prefix while no request is queued or running")
         n = len(tokens) // PAGE * PAGE
         if n >= min(self.max_seq_len, self._kv_pages * PAGE):
             raise ValueError("the prefix leaves no room: it exceeds max_seq_len or the KV cache")
-        self.kv.close(_PREFIX)
-        self._prefix = []
-        self.scheduler.kv_capacity = self._kv_pages * PAGE - n
-        self.runner.prefix_len.fill_(n)
+        self._drop_prefix()
         if n == 0:
             return 0
-        self.kv.open(_PREFIX)
-        pages = self.kv.reserve(_PREFIX, n).pages
-        step = self.scheduler.budget
-        for at in range(0, n, step):
-            self.runner.prefill([list(tokens[at:min(n, at + step)])], [at], [pages])
+        try:
+            self.kv.open(_PREFIX)
+            pages = self.kv.reserve(_PREFIX, n).pages
+            step = self.scheduler.budget
+            for at in range(0, n, step):
+                self.runner.prefill([list(tokens[at:min(n, at + step)])], [at], [pages])
+        except BaseException:
+            self._drop_prefix()
+            raise
         self.kv.seqs[_PREFIX].length = n
+        self.scheduler.kv_capacity = self._kv_pages * PAGE - n
+        self.runner.prefix_len.fill_(n)
         self._prefix = list(tokens[:n])
         return n
+
+    def _drop_prefix(self) -> None:
+        self.kv.close(_PREFIX)
+        self._prefix = []
+        self.scheduler.kv_capacity = self._kv_pages * PAGE
+        self.runner.prefix_len.fill_(0)
 
     # ------------------------------------------------------------ requests
     def add_request(self, prompt: list[int], params: SamplingParams | None = None,

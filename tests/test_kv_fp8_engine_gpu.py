@@ -219,3 +219,33 @@ def test_a_prefix_over_half_the_cache_serves_requests_together():
         eng.step()
     _check_status()
     assert eng.kv.alloc.free == 24
+
+
+def test_a_shared_prefix_that_cannot_be_set_leaves_the_engine_without_one():
+    from swarm_inference_lab_b200.engine.engine import SamplingParams
+    from swarm_inference_lab_b200.engine.kv_cache import OutOfPages
+    eng = _tiny(max_batch=8, max_seq_len=512, kv_pages=64, kv_dtype="fp8")
+    prefix = _prompts([200])[0]
+    prefill = eng.runner.prefill
+
+    def broken(*a, **kw):
+        raise RuntimeError("prefill failed")
+
+    for how in ("pages", "prefill"):
+        assert eng.set_shared_prefix(prefix) == 192
+        if how == "pages":
+            eng.kv.open("x")
+            eng.kv.reserve("x", 61 * PAGE)
+            with pytest.raises(OutOfPages):
+                eng.set_shared_prefix(prefix + prefix)
+            eng.kv.close("x")
+        else:
+            eng.runner.prefill = broken
+            with pytest.raises(RuntimeError, match="prefill failed"):
+                eng.set_shared_prefix(prefix)
+            eng.runner.prefill = prefill
+        assert eng.kv.alloc.free == 64 and not eng.kv.seqs
+        assert eng.scheduler.kv_capacity == 64 * PAGE and int(eng.runner.prefix_len) == 0
+        out, _ = eng.generate([prefix + [1]], SamplingParams(max_new_tokens=3))
+        assert len(out[0].token_ids) == 3 and eng.kv.alloc.free == 64
+    _check_status()
