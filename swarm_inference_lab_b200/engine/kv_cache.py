@@ -164,7 +164,8 @@ class PagedKVCache:
 
     def fork_prefix(self, src: str, dst: str, tokens: int) -> SeqPages:
         """Open ``dst`` on the whole pages of the first ``tokens`` tokens of ``src``, shared, not
-        copied: nobody writes a full page again, so both sequences may go on appending."""
+        copied: appending never writes a full page again, so both sequences may go on
+        (:meth:`truncate` copies the page that it makes writable)."""
         s = self.seqs[src]
         if dst in self.seqs:
             raise KeyError(f"sequence {dst} already open")
@@ -176,9 +177,19 @@ class PagedKVCache:
         return self.seqs[dst]
 
     def truncate(self, seq_id: str, length: int) -> None:
-        """Roll a sequence back to ``length`` tokens, releasing unused whole pages."""
+        """Roll a sequence back to ``length`` tokens, releasing unused whole pages.  A page that is
+        kept in part, and that other sequences share, is copied first: the sequence writes its rest
+        again (:class:`OutOfPages` if there is none for the copy; nothing has changed then)."""
         s = self.seqs[seq_id]
         keep = self.pages_for(length)
+        if length < s.length and length % PAGE and self.alloc.refcount(s.pages[keep - 1]) > 1:
+            old, (new,) = s.pages[keep - 1], self.alloc.alloc(1)
+            for t in (self.k, self.v, self.scales):
+                if t is not None:
+                    raw = t.view(torch.uint8)   # (indexing is not defined for every cache type)
+                    raw[:, new] = raw[:, old]
+            s.pages[keep - 1] = new
+            self.alloc.release([old])
         if keep < len(s.pages):
             self.alloc.release(s.pages[keep:])
             del s.pages[keep:]

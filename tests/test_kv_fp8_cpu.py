@@ -203,3 +203,43 @@ def test_a_request_on_a_shared_prefix_is_charged_its_own_pages():
         sch.admit(SeqRequest("odd", list(range(200)), 5, 99, shared_tokens=100))
     with pytest.raises(ValueError, match="shared"):
         sch.admit(SeqRequest("all", list(range(128)), 5, 99, shared_tokens=192))
+
+
+@pytest.mark.parametrize("kv_dtype", ["bf16", "fp8"])
+def test_truncating_a_fork_into_a_shared_page_copies_it(kv_dtype):
+    """A sequence that is rolled back below the end of a page that it shares writes the page's rest again:
+    into a copy of its own."""
+    from swarm_inference_lab_b200.engine.kv_cache import OutOfPages, PagedKVCache
+    kv = PagedKVCache(2, 2, 5, "cpu", kv_dtype=kv_dtype)
+    raw = (lambda t: t.view(torch.uint8)) if kv_dtype == "fp8" else (lambda t: t.view(torch.int16))
+    for t in (kv.k, kv.v):
+        raw(t).copy_(torch.randint(0, 100, raw(t).shape, generator=torch.Generator().manual_seed(1)))
+    if kv.scales is not None:
+        kv.scales.copy_(torch.randint(100, 150, kv.scales.shape, generator=torch.Generator().manual_seed(2)))
+    kv.open("p")
+    kv.reserve("p", 128)
+    kv.seqs["p"].length = 128
+    old = list(kv.seqs["p"].pages)
+    q = kv.fork_prefix("p", "q", 128)
+    kv.truncate("q", 128)
+    assert q.pages == old                                                          # nothing to write to
+    kv.truncate("q", 70)
+    assert q.length == 70 and q.pages[0] == old[0] and q.pages[1] not in old
+    for t in (raw(kv.k), raw(kv.v)) + ((kv.scales,) if kv.scales is not None else ()):
+        assert torch.equal(t[:, q.pages[1]], t[:, old[1]])
+    assert kv.alloc.refcount(old[0]) == 2 and kv.alloc.refcount(old[1]) == 1 and kv.alloc.free == 2
+    copy = q.pages[1]
+    kv.truncate("q", 65)
+    assert q.pages == [old[0], copy]                                               # its own by now
+    kv.truncate("q", 64)
+    assert q.pages == [old[0]] and kv.alloc.free == 3
+    kv.open("z")
+    kv.reserve("z", 192)
+    with pytest.raises(OutOfPages):
+        kv.truncate("q", 30)                                                       # no page for the copy
+    assert q.pages == [old[0]] and q.length == 64 and kv.alloc.refcount(old[0]) == 2
+    kv.close("z")
+    kv.truncate("q", 0)
+    assert q.pages == [] and q.length == 0 and kv.seqs["p"].pages == old
+    kv.close("p"), kv.close("q")
+    assert kv.alloc.free == 5
