@@ -146,6 +146,8 @@ def run_command(model: str, prompt: str = typer.Option(None, "--prompt"),
     if kv_dtype != "bf16" and require_distributed:
         raise typer.BadParameter("kv-dtype fp8 is for this box's engine, not a distributed run")
     cfg, res = _resolve_model(model)
+    if kv_dtype == "fp8" and cfg.mla:
+        raise typer.BadParameter("kv-dtype fp8 is for caches of K and V heads, not MLA latent rows")
     ckpt = _checkpoint_dir(model, res)
     tokenizer = None
     if ckpt is not None:

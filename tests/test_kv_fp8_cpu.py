@@ -243,3 +243,11 @@ def test_truncating_a_fork_into_a_shared_page_copies_it(kv_dtype):
     assert q.pages == [] and q.length == 0 and kv.seqs["p"].pages == old
     kv.close("p"), kv.close("q")
     assert kv.alloc.free == 5
+
+
+def test_cli_refuses_an_e4m3_cache_for_a_model_of_latent_rows():
+    from typer.testing import CliRunner
+    from swarm_inference_lab_b200.cli import app
+    for args in ([], ["--dry-run"]):
+        r = CliRunner().invoke(app, ["run", "tiny-mla-gpu", "--kv-dtype", "fp8", "--prompt", "x", *args])
+        assert r.exit_code == 2 and "kv-dtype" in r.output, (r.exit_code, r.output, r.exception)
