@@ -249,3 +249,107 @@ def test_a_shared_prefix_that_cannot_be_set_leaves_the_engine_without_one():
         out, _ = eng.generate([prefix + [1]], SamplingParams(max_new_tokens=3))
         assert len(out[0].token_ids) == 3 and eng.kv.alloc.free == 64
     _check_status()
+
+
+def _served(eng, prompt, n):
+    """Tokens of one request served alone, and the logits that each was taken from."""
+    from swarm_inference_lab_b200.engine.engine import SamplingParams
+    logits, seen = eng.model.logits, []
+
+    def keep(h, fb):
+        seen.append(logits(h, fb))
+        return seen[-1]
+
+    eng.model.logits = keep
+    try:
+        out = eng.generate([prompt], SamplingParams(max_new_tokens=n))[0][0].token_ids
+    finally:
+        eng.model.logits = logits
+    return out, [x[:1].clone() for x in seen[-n:]]
+
+
+@pytest.mark.parametrize("kv_dtype", ["fp8", "bf16"])
+def test_requests_on_a_shared_prefix_are_those_of_an_engine_without_one(kv_dtype):
+    """An engine whose prefill budget is the prefix's length computes a prompt's first 192 tokens in one
+    call, as the engine with a shared prefix did beforehand, and the rest in another: every shape is the
+    same, so tokens and logits must be, bit for bit.  A second prefix of another length, a request that
+    does not share, and one that is the prefix alone go through the same engine."""
+    kw = dict(max_batch=8, max_seq_len=512, kv_pages=64, kv_dtype=kv_dtype, use_cuda_graphs=False)
+    first, second = _prompts([200])[0], _prompts([320, 330])[1]
+    sharing = _tiny(prefill_token_budget=320, **kw)
+    for prefix, n in ((first, 192), (second, 320)):
+        plain = _tiny(prefill_token_budget=n, **kw)
+        assert sharing.set_shared_prefix(prefix) == n
+        seen = []
+        for tail in (1, 70, 33):
+            prompt = prefix[:n] + _prompts([tail])[0]
+            (a, la), (b, lb) = _served(sharing, prompt, 4), _served(plain, prompt, 4)
+            assert a == b and len(la) == 4 and all(torch.equal(x, y) for x, y in zip(la, lb))
+            seen += la
+        for prompt in (_prompts([20])[0], prefix[:n]):
+            (a, la), (b, lb) = _served(sharing, prompt, 4), _served(plain, prompt, 4)
+            assert a == b and all(torch.equal(x, y) for x, y in zip(la, lb))
+        assert not any(torch.equal(x, y) for x, y in zip(seen, seen[4:]))
+    _check_status()
+
+
+def test_a_decode_batch_on_a_prefix_that_is_attended_apart():
+    """The hidden states of a decode step through the shared-prefix operator against those of the same
+    step row by row: both attend to the same rows and round each attention output to bf16, so they differ
+    by roundings, and another prefix (whose hidden states are computed for comparison) changes them by the
+    size of the attention itself.  An eighth of that change is far above the roundings (2^-8 per output
+    and layer) and far below any row or page read wrongly.  With graphs the tokens are the same, also
+    after the prefix was replaced by one of another length."""
+    from swarm_inference_lab_b200.engine.engine import SamplingParams
+    kw = dict(max_batch=64, max_seq_len=4160, kv_pages=1600, kv_dtype="fp8")
+    eager, graphs = _tiny(use_cuda_graphs=False, **kw), _tiny(**kw)
+    assert 64 * 2 * eager.runner.max_pages > 8192              # (attended apart from here on)
+    texts = _prompts([1100, 1500, 1500])
+    tails = _prompts([3 + i % 7 for i in range(50)])
+    for text, other in ((texts[0], texts[1]), (texts[1], texts[2])):
+        n = eager.set_shared_prefix(text)
+        assert n == len(text) // PAGE * PAGE == graphs.set_shared_prefix(text)
+        rids = [eager.add_request(text[:n] + t, SamplingParams(max_new_tokens=4)) for t in tails]
+        eager.step()
+        reqs = [eager.scheduler.running[r] for r in rids]
+        ids, at = [r.output[-1] for r in reqs], [r.context_len - 1 for r in reqs]
+        pages = [list(eager.kv.seqs[r].pages) for r in rids]
+
+        def hidden(pages, shared):
+            dg = eager.runner.graph_for(64, shared=shared)
+            eager.runner.stage_decode_inputs(dg, ids, at, pages)
+            return eager.model.forward_hidden(dg.fb, eager.kv)[:50].float()
+
+        together, alone = hidden(pages, True), hidden(pages, False)
+        _check_status()
+        eager.kv.open("other")
+        instead = eager.kv.reserve("other", n).pages
+        eager.runner.prefill([other[:n]], [0], [instead])
+        changed = hidden([instead + p[n // PAGE:] for p in pages], False)
+        eager.kv.close("other")
+        change = (changed - alone).norm(dim=1)
+        assert ((together - alone).norm(dim=1) < change / 8).all()
+        for r in rids:
+            eager.cancel(r)
+        outs = [[o.token_ids for o in e.generate([text[:n] + t for t in tails], SamplingParams(max_new_tokens=4))[0]]
+                for e in (eager, graphs)]
+        _check_status()
+        assert outs[0] == outs[1] and any(shared for _, _, shared in graphs.runner.graphs)
+
+
+@pytest.mark.parametrize("moe", [False, True])
+def test_sampled_requests_on_a_shared_prefix(moe):
+    """Drawn tokens are the same from run to run, with and without graphs, in a dense and a mixture model."""
+    from swarm_inference_lab_b200.engine.engine import SamplingParams
+    kw = dict(moe=moe, max_batch=8, max_seq_len=512, kv_pages=64, kv_dtype="fp8")
+    prefix = torch.randint(0, 2048, (200,), generator=torch.Generator().manual_seed(1)).tolist()
+    prompts = [prefix[:192] + [i, 7, 9][:1 + i % 3] for i in range(4)]
+    params = SamplingParams(max_new_tokens=6, temperature=0.8, top_k=50, repetition_penalty=1.1, seed=5)
+    got = []
+    for graphs in (True, True, False):
+        eng = _tiny(use_cuda_graphs=graphs, **kw)
+        assert eng.set_shared_prefix(prefix) == 192
+        got.append([o.token_ids for o in eng.generate(prompts, params)[0]])
+        _check_status()
+        assert any(shared and sampled for _, sampled, shared in eng.runner.graphs)
+    assert got[0] == got[1] == got[2] and all(len(t) == 6 for t in got[0])
