@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, 4) rope_kv_write_fp8_kernel(const Wr
     if (nw != nullptr) {
       double ss = 0.0;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) ss += static_cast<double>(x[j] * x[j]);
+      for (int j = 0; j < 16; ++j) ss = fma(static_cast<double>(x[j]), static_cast<double>(x[j]), ss);
 #pragma unroll
       for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
       const double r = rsqrt(ss * (1.0 / kKvDim) + a.eps);
