@@ -15,10 +15,13 @@
 // small kernel joins them in page order.  Nothing is shared between calls, there are no atomics, and
 // results do not change from run to run.
 //
-// Measured (device time of both kernels): 32 sequences of 2048 tokens, 32/8 heads (136 MB), 31.8 us, of
-// which the pages take 27 (5.0 TB/s, bound by memory) and the join 4-5; 61 ragged sequences up to 8191
-// tokens, 32/4 heads, 24 us, against 72 with a CTA to a unit and 35 with four; one of 200 tokens 5.3 us,
-// bound by the chain of launch, lengths, page ids, page and join.
+// Measured (device time of both kernels): 32 sequences of 2048 tokens, 32/8 heads (136 MB), 32.0 us, of
+// which the pages take 27 (5.0 TB/s) and the join 4-5.  No unit is full in the page loop (DRAM at 0.71 of
+// the copy rate in a profile of it alone, issue slots 39%, ALU 41%): 15 warps to an SM, at 128 registers,
+// wait for pages and for their own chain of load, convert, MMA and softmax.  61 ragged sequences up to
+// 8191 tokens, 32/4 heads, 24.5 us, against 72 with a CTA to a unit and 35 with four; the same work takes
+// 32 equal sequences 28.5 us with a CTA to a unit: equal shares cost them the join.  One of 200 tokens
+// 5.5 us, bound by the chain of launch, lengths, page ids, page and join.
 //
 // Arithmetic.  Codes become f16 fragments exactly (e4m3 is a subset of f16); q is scaled per row by a
 // power of two into f16's range.  The value scale joins the exponent: with s the score in the exp2
@@ -53,7 +56,9 @@ constexpr int kStageBytes = 2 * kSideBytes;
 constexpr int kScaleBytes = 2 * kKvPage;               // both sides' scales of one page and head
 constexpr int kWarps = 4;                              // consumer warps
 constexpr int kThreads = (kWarps + 1) * 32;
-// A context of up to so many pages (by the block table's width) is one CTA's work.
+// A context of up to so many pages is one CTA's work.  That goes by the block table's width, which the
+// host knows, not by the lengths: one sequence of 200 tokens takes 5.5 us with 4 columns and 7.8 with 16 to
+// 512, 32 of them with 8 KV heads 7.6 and 12.6.
 constexpr int kWholePages = 8;
 // (Geometric mean over 20 decode cases, 1 to 61 sequences, 1 to 20000 tokens: kMinWork 5, 8, 14: 10.6,
 // 10.7, 11.6 us; kUnitCost 1, 3, 6: 11.1, 10.6, 10.6; kWholePages 8, 32: 10.6, 10.6.)

@@ -21,7 +21,7 @@
 // last token reaches a product; a token marked not finite gets NaN keys (masked where it is not
 // seen) and zero values.  P is rounded to bf16; m, l, S and O are fp32.
 //
-// Measured: 1000 queries on 31000 tokens, 32/4 heads, 755 us (660 TFLOP/s); 558 us with the unpacking's
+// Measured: 1000 queries on 31000 tokens, 32/4 heads, 755-780 us (640-660 TFLOP/s); 558 us with the unpacking's
 // work left out, so its issue slots are what the other warps miss, and the chain S, softmax, PV of a
 // tile bounds the rest (S_X of the next tile overwrites P_X, so it waits for PV_X).  Steps of 64 keys with
 // two S buffers avoid that wait but read Q twice as often and took 839 us.
@@ -72,7 +72,9 @@ static_assert(128 * (kRegsWg0 + kQT * kRegsSoftmax + kRegsUnpack) <= kThreads * 
 constexpr int kShortRows = 32;
 // Pages (of sequences and KV heads, by the block table's width) up to which a shared prefix is not
 // attended apart: reading 8192 takes some 33 us, 12 sequences of 6400 tokens and 8 KV heads (9700
-// pages) with the prefix apart 37 us.
+// pages) with the prefix apart 37 us.  Contexts much shorter than their table lose by it: 32 sequences on
+// 64 shared tokens and 136 own, 8 KV heads, take 22.8 us apart (64 columns) and 12.5 row by row, on 2048
+// shared ones 26.7 and 26.5.
 constexpr int64_t kUnsharedPages = 8192;
 constexpr int kTmemCols = 512;
 constexpr uint32_t kColO = 256;                // O_X at kColO + 128 X; S_X / P_X at 128 X
@@ -799,7 +801,7 @@ at::Tensor paged_decode_shared_fp8(const at::Tensor& q, const at::Tensor& k_cach
   if (B == 0) return out;
   c10::cuda::CUDAGuard guard(q.device());
   const int64_t Hkv = k_cache.size(1);
-  // Where every sequence reading all its pages takes no longer than the two more launches.
+  // Where every sequence reading all pages of its table's width takes no longer than the two more launches.
   if (B * Hkv * block_table.size(1) <= kUnsharedPages) {
     attn_fp8(what, q, k_cache, v_cache, scales, block_table, seq_lens, nullptr, 1, out, scale,
              prefix_len.data_ptr<int>(), nullptr, nullptr, 0, status);

@@ -1,10 +1,10 @@
 // Writing the e4m3 KV cache (per-head RMSNorm, RoPE and quantisation in one pass) and reading
 // rows of it back as bf16.  Format: sil/kv_fp8.cuh.
 //
-// Between the bf16 inputs and the single rounding of each output all is fp32: the norm
-// x * rsqrt(mean x^2 + eps) * w, the rotation (a, b) -> (a c - b s, b c + a s) of dims d and
-// d + 64, and the quantisation; a key keeps its remainders beside (see rotate_sticky).  Both kernels
-// are bound by memory traffic.
+// Between the bf16 inputs and the single rounding of each output queries are fp32: the norm
+// x * rsqrt(mean x^2 + eps) * w, the rotation (a, b) -> (a c - b s, b c + a s) of dims d and d + 64.
+// A key keeps its remainders beside (rotate_sticky), and its norm's sum and factor are fp64.  Both
+// kernels are bound by memory traffic.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -114,8 +114,8 @@ __device__ __forceinline__ void quantize_head(const WriteArgs& a, const float (&
 // One group of eight lanes takes kPer heads of a token: their loads are in flight together and share
 // the token's angles.  Traffic is all that counts, so four CTAs to an SM, at 64 registers: with the 68
 // and 108 that one and four heads would like, 16384 tokens of 32/8 heads took 110 and 140 us, with one
-// and two heads at 64 they take 94 and 79 us (5.0 TB/s, 73% of the copy rate); 4000 tokens with norms
-// 29 and 32 us.
+// and two heads at 64 they took 94 and 79 us (4000 tokens with norms 29 and 32).  Since the keys'
+// remainders are added up before the rounding, two heads take 82 us (4.6 TB/s, 71% of the copy rate).
 template <int kPer>
 __global__ void __launch_bounds__(kThreads, 4) rope_kv_write_fp8_kernel(const WriteArgs a) {
   pdl_trigger();

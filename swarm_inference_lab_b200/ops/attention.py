@@ -107,8 +107,9 @@ def paged_decode_shared_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
 
     ``prefix_len`` (int32 [1], on the device) is how many tokens are shared.  Every sequence of at
     least that length holds the same page ids in the prefix's whole pages (the device status is
-    raised if one does not); shorter ones are read through their own row alone.  Small batches read
-    the prefix once per sequence all the same, where that takes no longer."""
+    raised if one does not); shorter ones are read through their own row alone.  Where batch, KV
+    heads and columns of the block table multiply to 8192 or less, the prefix is read once per
+    sequence all the same."""
     return ext().paged_decode_shared_fp8(q, k_cache, v_cache, kv_scales, block_table, seq_lens,
                                          prefix_len, out, SCALE_128 if scale is None else scale,
                                          get_workspace(q.device).status)

@@ -55,7 +55,9 @@ def rope_kv_write_fp8(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.T
 
     ``k_cache`` / ``v_cache`` are e4m3 ``[pages, Hkv, 64, 128]``, ``kv_scales`` uint8
     ``[pages, Hkv, 2, 64]`` (one power-of-two scale per token, head and side; see
-    :mod:`.kv_fp8`).  All arithmetic is fp32 and each output is rounded once.  The rotated
+    :mod:`.kv_fp8`).  Queries are computed in fp32 and rounded once; a key's norm is computed in fp64
+    and its rotation keeps what it rounds off, so that its codes are those of the exact values (none
+    wrong among 84 million in an emulation; rounding to fp32 first: 96).  The rotated
     queries go to ``q_out`` [T, Hq, 128], or back into ``qkv`` without it; returned either way.
     A negative slot skips the token's cache write (its queries are rotated all the same); the
     other slots must differ from one another.  A slot past the cache, or a position outside
