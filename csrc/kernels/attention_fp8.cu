@@ -26,11 +26,11 @@
 // Arithmetic.  Codes become f16 fragments exactly (e4m3 is a subset of f16); q is scaled per row by a
 // power of two into f16's range.  The value scale joins the exponent: with s the score in the exp2
 // domain and e the exponent of V's scale,
-//   P = 2^(s + e - m),   O = sum P v8,   l = sum P 2^-e,   m = running max of s + e,   out = O / l,
+//   P = 2^(s + e - m),   O = sum P v8,   l = sum P 2^-e,   m = running max of s + e - 15,   out = O / l,
 // which is softmax(s) V for any m, so parts with other references (a prefix's, whose m is max s) join by
-// the same formula.  With m the maximum of the pages' own s + e, P <= 1 reaches 1 whatever the scales, so
-// f16 holds it: 2^-12 relative, and P v8 below 2^-14 of the largest to 2^-25 of it.  S, m, l and O are fp32
-// (a token counts as nothing where its s + e is 126 below the largest).
+// the same formula.  With m from the pages' own s + e, P reaches 2^15 whatever the scales, which uses f16's
+// whole range: P v8 down to 2^-29 of the largest is held to 2^-12 of itself, smaller to 2^-40 of the largest.
+// S, m, l and O are fp32.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp16.h>
@@ -179,6 +179,9 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+
+// log2 of the largest P: f16 ends at 2^16.
+constexpr float kTop = 15.f;
 
 // Joins partials (m_i, l_i, o_i) of one row: rescaling factor of a part, 0 where there is none.
 __device__ __forceinline__ float part_factor(float m, float M) {
@@ -571,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, kTiles == 1 ? 3 : 2)
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          const float m_new = fmaxf(m_r[u][j], mx);
+          const float m_new = fmaxf(m_r[u][j], mx - kTop);
           m_use[j] = m_new == -INFINITY ? 0.f : m_new;
           alpha[j] = ex2_approx(m_r[u][j] - m_use[j]);
           m_r[u][j] = m_new;

@@ -115,7 +115,7 @@ __device__ __forceinline__ void quantize_head(const WriteArgs& a, const float (&
 // the token's angles.  Traffic is all that counts, so four CTAs to an SM, at 64 registers: with the 68
 // and 108 that one and four heads would like, 16384 tokens of 32/8 heads took 110 and 140 us, with one
 // and two heads at 64 they took 94 and 79 us (4000 tokens with norms 29 and 32).  Since the keys'
-// remainders are added up before the rounding, two heads take 82 us (4.6 TB/s, 71% of the copy rate).
+// remainders are added up before the rounding, two heads take 81 us (4.7 TB/s, 71% of the copy rate).
 template <int kPer>
 __global__ void __launch_bounds__(kThreads, 4) rope_kv_write_fp8_kernel(const WriteArgs a) {
   pdl_trigger();
